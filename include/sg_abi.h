@@ -397,6 +397,15 @@ int sg_paged_attention(const sg_kv_cache* cache, const uint16_t* q, long long q_
                        const int32_t* page_table, int table_width, const int32_t* lengths, float scale,
                        uint16_t* out, void* work, long long work_bytes, void* stream);
 
+/* The same with the table row of each row of q: row b attends the tokens of page_table
+ * [table_rows, table_width] row rows[b] (row b when rows is NULL; table_rows >= B
+ * then), so that tokens of one sequence share its table row.  A row outside the table is zero and, where its
+ * length is not 0 or less (padding), recorded (SG_ERR_CAPACITY). */
+int sg_paged_attention_rows(const sg_kv_cache* cache, const uint16_t* q, long long q_stride, int B, int q_heads,
+                            const int32_t* page_table, int table_rows, int table_width, const int32_t* rows,
+                            const int32_t* lengths, float scale, uint16_t* out, void* work,
+                            long long work_bytes, void* stream);
+
 /* ------------------------------------------ expert-parallel exchange (e)
  * The dispatch / combine all-to-alls of one expert-parallel layer over
  * NVLink peer memory, one process per GPU, R <= 8 ranks in lockstep.  No

@@ -37,6 +37,7 @@ EXPORTED_SYMBOLS = (
     "sg_ep_ipc_close", "sg_ep_send", "sg_ep_wait_inbox", "sg_ep_send_back", "sg_ep_wait_back",
     "sg_ep_set_wait_limit",
     "sg_add_rms_norm", "sg_quantize_fp8", "sg_fp8_linear", "sg_append_kv", "sg_paged_attention_work_bytes", "sg_paged_attention",
+    "sg_paged_attention_rows",
 )
 
 
@@ -138,6 +139,7 @@ def load() -> ctypes.CDLL:
         "sg_append_kv": (I32, [KV, P, LL, P, LL, P, LL, I32, I32, P, I32, I32, P, P, P, I32, I32, P, P, F, P, P]),
         "sg_paged_attention_work_bytes": (LL, [KV, I32, I32]),
         "sg_paged_attention": (I32, [KV, P, LL, I32, I32, P, I32, P, F, P, P, LL, P]),
+        "sg_paged_attention_rows": (I32, [KV, P, LL, I32, I32, P, I32, I32, P, P, F, P, P, LL, P]),
     }
     for name, (res, args) in sigs.items():
         fn = getattr(lib, name)
@@ -162,7 +164,7 @@ def native():
             raise ImportError(
                 f"{e}: build the extension first (python -m preemptlm_b200.build); there is no CPU fallback") from e
         names = ("sg_add_rms_norm", "sg_quantize_fp8", "sg_fp8_linear", "sg_append_kv", "sg_paged_attention_work_bytes",
-                 "sg_paged_attention")
+                 "sg_paged_attention_rows")
         _native.bind({n: ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in names})
         _binding = _native
     return _binding

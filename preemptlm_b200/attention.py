@@ -54,16 +54,17 @@ class PagedAttention:
         """One step of T tokens.  x [T, H] bf16 is added to the residual
         stream; token t is the positions[t]-th of page_table row rows[t] (row
         t if None; several tokens of a row in one call see each other's keys
-        up to their own place).  Returns (the attention's output [T, H], the
-        new residual [T, H])."""
+        up to their own place).  A negative position marks a padding token,
+        whose row may be anything.  A row outside the table attends nothing;
+        ``ops.device_status`` reports it.  Returns (the attention's output [T,
+        H], the new residual [T, H])."""
         T, D, kv = x.shape[0], self.cache.head_dim, self.cache.kv_heads
         y8, scales, residual = ops.add_rms_norm_fp8(x, self.norm, residual=residual, eps=self.eps)
         qkv = ops.fp8_linear(y8, scales, *self.qkv).view(T, self.q_heads + 2 * kv, D)
         q, k, v = qkv.split([self.q_heads, kv, kv], dim=1)
         q = ops.append_kv(self.cache, q, k, v, page_table, positions, self.rope, rows=rows, q_weight=self.q_norm,
                           k_weight=self.k_norm, eps=self.eps)
-        table = page_table if rows is None else page_table.index_select(0, rows)
-        o = ops.paged_attention(self.cache, q, table, positions + 1)
+        o = ops.paged_attention(self.cache, q, page_table, positions + 1, rows=rows)
         o8, scales = ops.quantize_fp8(o.view(T, self.q_heads * D))
         return ops.fp8_linear(o8, scales, *self.out), residual
 

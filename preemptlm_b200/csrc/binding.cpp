@@ -21,7 +21,7 @@ decltype(&sg_quantize_fp8) p_quantize_fp8;
 decltype(&sg_fp8_linear) p_fp8_linear;
 decltype(&sg_append_kv) p_append_kv;
 decltype(&sg_paged_attention_work_bytes) p_work_bytes;
-decltype(&sg_paged_attention) p_paged_attention;
+decltype(&sg_paged_attention_rows) p_paged_attention;
 
 constexpr int64_t BLOCK = 128;  // values that share an 8-bit row's scale
 
@@ -265,26 +265,28 @@ PyObject* append_kv(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
-// paged_attention(cache address, device, q, page_table, lengths, scale): out
+// paged_attention(cache address, device, q, page_table, lengths, scale, rows): out
 PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  if (!want(n, 6, "paged_attention")) return nullptr;
+  if (!want(n, 7, "paged_attention")) return nullptr;
   return guarded([&]() -> PyObject* {
     const sg_kv_cache* c = cache_at(a[0]);
     const int64_t device = device_of(a[1]), D = c->head_dim;
     const at::Tensor q = heads(a[2], "q", D, device);
     const int64_t B = q.size(0), Hq = q.size(1);
-    const at::Tensor table = page_table(a[3], B, device), lengths = vector_int32(a[4], "lengths", B, device);
+    const at::Tensor table = page_table(a[3], is_none(a[6]) ? B : -1, device), lengths = vector_int32(a[4], "lengths", B, device);
     const double scale = PyFloat_AsDouble(a[5]);
     if (scale == -1.0 && PyErr_Occurred()) throw Raised();
+    at::Tensor row_of;
+    if (!is_none(a[6])) row_of = vector_int32(a[6], "rows", B, device);
     const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(device));
     const long long bytes = p_work_bytes(c, checked_int(B), checked_int(Hq));
     if (bytes < 0) return status(static_cast<int>(bytes));
     at::Tensor out = at::empty({B, Hq, D}, q.options());
     at::Tensor work = at::empty({bytes}, q.options().dtype(at::kByte));
     const int st = p_paged_attention(c, at_ptr<uint16_t>(q), q.stride(0), checked_int(B), checked_int(Hq),
-                                     at_ptr<int32_t>(table), checked_int(table.size(1)), at_ptr<int32_t>(lengths),
-                                     static_cast<float>(scale), at_ptr<uint16_t>(out), work.data_ptr(), bytes,
-                                     stream(device));
+                                     at_ptr<int32_t>(table), checked_int(table.size(0)), checked_int(table.size(1)),
+                                     at_ptr<int32_t>(row_of), at_ptr<int32_t>(lengths), static_cast<float>(scale),
+                                     at_ptr<uint16_t>(out), work.data_ptr(), bytes, stream(device));
     return st != SG_OK ? status(st) : wrap(out);
   });
 }
@@ -299,7 +301,7 @@ PyObject* bind(PyObject*, PyObject* names) {
                  {"sg_fp8_linear", reinterpret_cast<void**>(&p_fp8_linear)},
                  {"sg_append_kv", reinterpret_cast<void**>(&p_append_kv)},
                  {"sg_paged_attention_work_bytes", reinterpret_cast<void**>(&p_work_bytes)},
-                 {"sg_paged_attention", reinterpret_cast<void**>(&p_paged_attention)}};
+                 {"sg_paged_attention_rows", reinterpret_cast<void**>(&p_paged_attention)}};
   if (!PyDict_Check(names)) {
     PyErr_SetString(PyExc_TypeError, "bind takes a dict of addresses");
     return nullptr;

@@ -201,7 +201,9 @@ struct Args {
   const uint16_t* q;
   long long q_stride;
   int B, q_heads, group, sub, width;  // sub: parts of at most 16 (8) heads that a group is split into
-  const int32_t* table;
+  const int32_t* table;  // [table_rows, width]
+  int table_rows;
+  const int32_t* rows;  // [B] or null: row b's table row is b
   const int32_t* lengths;
   float scale_log2;  // softmax scale * log2(e)
   uint16_t* out;     // [B, q_heads, D]
@@ -317,9 +319,16 @@ struct Cursor {
   int b, h, k, len, slices;
 };
 
+__device__ __forceinline__ int table_row(const Args& a, int b) { return a.rows ? a.rows[b] : b; }
+__device__ __forceinline__ bool no_row(const Args& a, int b) {
+  return a.rows && static_cast<unsigned>(a.rows[b]) >= static_cast<unsigned>(a.table_rows);
+}
+
+// Tokens of row b that count; none if it has no row in the table.
 __device__ __forceinline__ int row_length(const Args& a, int b) {
   const int cap = a.width << a.c.page_shift;
-  return min(max(a.lengths[b], 0), cap);
+  const int len = min(max(a.lengths[b], 0), cap);
+  return no_row(a, b) ? 0 : len;
 }
 
 template <int SLICE>
@@ -349,7 +358,7 @@ __device__ __forceinline__ Item fetch(const Args& a, const Cursor& c, int lane) 
   it.page = -1;
   const int tok = it.tok + lane % SLICE;
   if (tok < c.len) {
-    it.page = *(a.table + static_cast<long long>(c.b) * a.width + (tok >> a.c.page_shift));
+    it.page = *(a.table + static_cast<long long>(table_row(a, c.b)) * a.width + (tok >> a.c.page_shift));
     if (it.page < 0 || it.page >= a.c.num_pages) {  // such tokens are masked; the host reads the status
       record(SG_ERR_CAPACITY);
       it.page = -1;
@@ -435,6 +444,7 @@ attention_kernel(const Args a) {
       a.prefix[b] = at;
       const int len = a.lengths[b];
       if (len > (a.width << a.c.page_shift)) record(SG_ERR_CAPACITY);
+      if (len > 0 && no_row(a, b)) record(SG_ERR_CAPACITY);
       at += (row_length(a, b) + SLICE - 1) / SLICE * heads;
     }
     if (threadIdx.x == 0) a.prefix[a.B] = per;
@@ -1071,18 +1081,20 @@ extern "C" long long sg_paged_attention_work_bytes(const sg_kv_cache* cache, int
   return rc == SG_OK ? bytes : rc;
 }
 
-extern "C" int sg_paged_attention(const sg_kv_cache* cache, const uint16_t* q, long long q_stride, int B, int q_heads,
-                                  const int32_t* page_table, int table_width, const int32_t* lengths, float scale,
-                                  uint16_t* out, void* work, long long work_bytes, void* stream) {
+extern "C" int sg_paged_attention_rows(const sg_kv_cache* cache, const uint16_t* q, long long q_stride, int B, int q_heads,
+                                       const int32_t* page_table, int table_rows, int table_width, const int32_t* rows,
+                                       const int32_t* lengths, float scale, uint16_t* out, void* work,
+                                       long long work_bytes, void* stream) {
   using namespace sg::attn;
   const long long need = sg_paged_attention_work_bytes(cache, B, q_heads);
   if (need < 0) return (int)need;
   Args a{};
   check_cache(cache, &a.c);
-  if (table_width < 0) return SG_ERR_INVALID_ARG;
+  if (table_rows < 0 || table_width < 0) return SG_ERR_INVALID_ARG;
   if (q_stride % 8 || q_stride < 0) return SG_ERR_SHAPE;
+  if (!rows && table_rows < B) return SG_ERR_INVALID_ARG;
   if (B == 0) return SG_OK;
-  if (!q || !lengths || !out || !work || (table_width > 0 && !page_table)) return SG_ERR_INVALID_ARG;
+  if (!q || !lengths || !out || !work || (table_rows > 0 && table_width > 0 && !page_table)) return SG_ERR_INVALID_ARG;
   if (misaligned16(q) || misaligned16(out) || misaligned16(work)) return SG_ERR_INVALID_ARG;
   if (work_bytes < need) return SG_ERR_CAPACITY;
   a.group = q_heads / a.c.kv_heads;
@@ -1091,10 +1103,17 @@ extern "C" int sg_paged_attention(const sg_kv_cache* cache, const uint16_t* q, l
   const long long longest = static_cast<long long>(table_width) << a.c.page_shift;
   if (longest > (1 << 30) || B * heads * ((longest + 15) / 16) > (1 << 30)) return SG_ERR_SHAPE;
   a.q = q; a.q_stride = q_stride; a.B = B; a.q_heads = q_heads; a.width = table_width;
-  a.table = page_table; a.lengths = lengths; a.scale_log2 = scale * 1.44269504f; a.out = out;
+  a.table = page_table; a.table_rows = table_rows; a.rows = rows; a.lengths = lengths; a.scale_log2 = scale * 1.44269504f; a.out = out;
   int dev = 0;
   SG_CUDA_TRY(cudaGetDevice(&dev));
   return by_format(cache->head_dim, cache->bits, half, [&](auto dim, auto fp8, auto hf) -> int {
     return launch_attention<dim.value, fp8.value, hf.value>(a, static_cast<uint8_t*>(work), dev, (cudaStream_t)stream);
   });
+}
+
+extern "C" int sg_paged_attention(const sg_kv_cache* cache, const uint16_t* q, long long q_stride, int B, int q_heads,
+                                  const int32_t* page_table, int table_width, const int32_t* lengths, float scale,
+                                  uint16_t* out, void* work, long long work_bytes, void* stream) {
+  return sg_paged_attention_rows(cache, q, q_stride, B, q_heads, page_table, B, table_width, nullptr, lengths, scale, out,
+                                 work, work_bytes, stream);
 }

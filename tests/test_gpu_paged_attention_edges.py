@@ -5,9 +5,10 @@ the ordinary cases."""
 import pytest
 import torch
 
-from preemptlm_b200 import ops
+from preemptlm_b200 import _abi, ops
 
-from .test_gpu_paged_attention import DEV, attend64, make_cache, make_table, rand
+from .test_gpu_decoder_layer import make
+from .test_gpu_paged_attention import BF, DEV, attend64, check_attention, make_cache, make_table, rand
 
 pytestmark = pytest.mark.gpu
 
@@ -29,3 +30,63 @@ def test_probabilities_keep_sixteen_bits(bits, D, heads, group):
     err = (got.double() - ref).abs()
     bound = ref.abs() * 2.0 ** -8 + mag * 2.0 ** -15
     assert bool((err <= bound).all()), float((err / bound).max())
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("D,heads,group", [(64, 2, 2), (128, 1, 16), (256, 2, 8)])
+def test_rows_of_the_table(bits, D, heads, group):
+    """Tokens that share table rows, in any order, equal the same call over a gathered table; a row outside the table is
+    zero, and recorded unless its token is padding."""
+    page, sequences = 16, 4
+    table, total = make_table([300, 40, 0, 700], page, 1)
+    cache = make_cache(total, heads, page, D, bits, 2)
+    rows = torch.tensor([3, 0, 0, 1, 3, 2, 3, 0, 1], dtype=torch.int32, device=DEV)
+    lengths = [700, 1, 300, 40, 33, 0, 16, 155, 17]
+    n = torch.tensor(lengths, dtype=torch.int32, device=DEV)
+    q = rand((len(lengths), heads * group, D), 5)
+    ops.device_status()
+    got = ops.paged_attention(cache, q, table, n, rows=rows)
+    assert torch.equal(got, ops.paged_attention(cache, q, table[rows.long()], n))
+    check_attention(got, *attend64(cache, q, table[rows.long()], lengths), bits)
+    assert ops.device_status() == 0
+    for outside in (-1, sequences, -(1 << 31), (1 << 31) - 1):
+        at, none = torch.tensor([0, 5, 8], device=DEV), torch.tensor([-7, 0, -1], dtype=torch.int32, device=DEV)
+        bad = rows.clone()
+        bad[at] = outside
+        padded = n.clone()
+        padded[at] = none
+        out = ops.paged_attention(cache, q, table, padded, rows=bad)
+        assert ops.device_status() == 0  # padding tokens
+        assert bool((out[at] == 0).all())
+        keep = [1, 2, 3, 4, 6, 7]
+        assert torch.equal(out[keep], got[keep])
+        out = ops.paged_attention(cache, q, table, n, rows=bad)
+        assert ops.device_status() == _abi.SG_ERR_CAPACITY
+        assert bool((out[at] == 0).all()) and torch.equal(out[keep], got[keep])
+    with pytest.raises(TypeError):
+        ops.paged_attention(cache, q, table, n, rows=rows.long())
+    with pytest.raises(TypeError):
+        ops.paged_attention(cache, q, table, n, rows=rows[:3])
+
+
+@pytest.mark.parametrize("padding_row", [-1, 2, 1 << 30])
+def test_block_with_padding_tokens(padding_row):
+    """A step padded to a fixed size, its padding tokens' rows outside the table: what the tokens alone give."""
+    att = make(256, 4, 2, 64, 64, 16, 8, BF)
+    table = torch.arange(8, device=DEV, dtype=torch.int32).view(2, 4)
+    x, r = rand((7, 256), 1), rand((7, 256), 2, 2.0)
+    rows = torch.tensor([0, 0, 1, 0, 1], dtype=torch.int32, device=DEV)
+    pos = torch.tensor([0, 1, 0, 2, 1], dtype=torch.int32, device=DEV)
+    live = torch.tensor([0, 1, 3, 4, 6], device=DEV)
+    want, _ = att(x[live], r[live], table, pos, rows)
+    all_rows = torch.full((7,), padding_row, dtype=torch.int32, device=DEV)
+    all_pos = torch.full((7,), -1, dtype=torch.int32, device=DEV)
+    all_rows[live], all_pos[live] = rows, pos
+    ops.device_status()
+    got, _ = att(x, r, table, all_pos, all_rows)
+    assert ops.device_status() == 0
+    assert torch.equal(got[live], want) and bool((got[[2, 5]] == 0).all())
+    all_pos[2] = 3  # a token without a sequence: left out and reported, the others as they were
+    got, _ = att(x, r, table, all_pos, all_rows)
+    assert ops.device_status() == _abi.SG_ERR_CAPACITY
+    assert torch.equal(got[live], want) and bool((got[[2, 5]] == 0).all())
