@@ -221,9 +221,9 @@ int64_t device_of(PyObject* o) {
   if (v == -1 && PyErr_Occurred()) throw Raised();
   return v;
 }
-at::Tensor page_table(PyObject* o, int64_t rows_wanted, int64_t device) {
+at::Tensor page_table(PyObject* o, int64_t rows_needed, int64_t device) {
   const at::Tensor& t = tensor(o, "page_table");
-  if (t.scalar_type() != at::kInt || t.dim() != 2 || (rows_wanted >= 0 && t.size(0) != rows_wanted) || !on(t, device))
+  if (t.scalar_type() != at::kInt || t.dim() != 2 || t.size(0) < rows_needed || !on(t, device))
     type_error("%s must be an int32 [rows, pages] tensor on the cache's device", "page_table");
   return t.contiguous();
 }
@@ -238,7 +238,7 @@ PyObject* append_kv(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int64_t T = q.size(0);
     if (k.size(0) != T || v.size(0) != T || k.size(1) != c->kv_heads || v.size(1) != c->kv_heads)
       value_error("k and v must have q's tokens and the cache's heads");
-    const at::Tensor table = page_table(a[5], -1, device), positions = vector_int32(a[6], "positions", T, device);
+    const at::Tensor table = page_table(a[5], 0, device), positions = vector_int32(a[6], "positions", T, device);
     at::Tensor rope, row_of, q_weight, k_weight;
     if (!is_none(a[8])) row_of = vector_int32(a[8], "rows", T, device);
     else if (table.size(0) < T) value_error("without rows, page_table needs a row for every token");
@@ -273,7 +273,7 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int64_t device = device_of(a[1]), D = c->head_dim;
     const at::Tensor q = heads(a[2], "q", D, device);
     const int64_t B = q.size(0), Hq = q.size(1);
-    const at::Tensor table = page_table(a[3], is_none(a[6]) ? B : -1, device), lengths = vector_int32(a[4], "lengths", B, device);
+    const at::Tensor table = page_table(a[3], is_none(a[6]) ? B : 0, device), lengths = vector_int32(a[4], "lengths", B, device);
     const double scale = PyFloat_AsDouble(a[5]);
     if (scale == -1.0 && PyErr_Occurred()) throw Raised();
     at::Tensor row_of;

@@ -454,7 +454,7 @@ def paged_attention(cache, q: torch.Tensor, page_table: torch.Tensor, lengths: t
     """Attention of new tokens over the paged cache (``sg_paged_attention_rows``):
     row b of q [B, q_heads, D] attends the first lengths[b] (int32) cached
     tokens of row ``rows[b]`` (int32; row b if None) of page_table int32 [rows,
-    pages]; query heads share key-value heads in consecutive groups.  scale
+    pages] (at least B rows if ``rows`` is None); query heads share key-value heads in consecutive groups.  scale
     defaults to D ** -0.5.  Returns bf16 [B, q_heads, D]; a row of length 0 is
     zero, and so is one outside the table.  The lengths stay on the device: a
     captured graph serves growing caches.  Several new tokens of one sequence

@@ -90,3 +90,22 @@ def test_block_with_padding_tokens(padding_row):
     got, _ = att(x, r, table, all_pos, all_rows)
     assert ops.device_status() == _abi.SG_ERR_CAPACITY
     assert torch.equal(got[live], want) and bool((got[[2, 5]] == 0).all())
+
+
+def test_table_with_more_rows_than_tokens():
+    """Append and attention take the same tables: a fixed one with a smaller step."""
+    page = 16
+    table, total = make_table([40, 40, 40, 40], page, 1)
+    cache = make_cache(total, 2, page, 128, 16, 2)
+    q, n = rand((2, 8, 128), 3), torch.tensor([33, 20], dtype=torch.int32, device=DEV)
+    got = ops.paged_attention(cache, q, table, n)
+    assert torch.equal(got, ops.paged_attention(cache, q, table[:2], n))
+    check_attention(got, *attend64(cache, q, table[:2], [33, 20]), 16)
+    with pytest.raises(TypeError):
+        ops.paged_attention(cache, q, table[:1], n)
+    att = make(256, 4, 2, 64, 64, 16, 8, BF)
+    table = torch.arange(8, device=DEV, dtype=torch.int32).view(4, 2)
+    x, r, pos = rand((2, 256), 1), rand((2, 256), 2, 2.0), torch.zeros(2, dtype=torch.int32, device=DEV)
+    want, _ = att(x, r, table[:2], pos)
+    got, _ = att(x, r, table, pos)
+    assert torch.equal(got, want)
