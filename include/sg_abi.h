@@ -400,10 +400,13 @@ int sg_paged_attention(const sg_kv_cache* cache, const uint16_t* q, long long q_
 /* The same with the table row of each row of q: row b attends the tokens of page_table
  * [table_rows, table_width] row rows[b] (row b when rows is NULL; table_rows >= B
  * then), so that tokens of one sequence share its table row.  A row outside the table is zero and, where its
- * length is not 0 or less (padding), recorded (SG_ERR_CAPACITY). */
+ * length is not 0 or less (padding), recorded (SG_ERR_CAPACITY).  So is a row
+ * longer than max_length (SG_ERR_SHAPE): with max_length = sg_append_kv's max_pos and
+ * lengths = positions + 1, a token that the append left out attends nothing;
+ * INT32_MAX: no such limit. */
 int sg_paged_attention_rows(const sg_kv_cache* cache, const uint16_t* q, long long q_stride, int B, int q_heads,
                             const int32_t* page_table, int table_rows, int table_width, const int32_t* rows,
-                            const int32_t* lengths, float scale, uint16_t* out, void* work,
+                            const int32_t* lengths, int max_length, float scale, uint16_t* out, void* work,
                             long long work_bytes, void* stream);
 
 /* ------------------------------------------ expert-parallel exchange (e)

@@ -139,7 +139,7 @@ def load() -> ctypes.CDLL:
         "sg_append_kv": (I32, [KV, P, LL, P, LL, P, LL, I32, I32, P, I32, I32, P, P, P, I32, I32, P, P, F, P, P]),
         "sg_paged_attention_work_bytes": (LL, [KV, I32, I32]),
         "sg_paged_attention": (I32, [KV, P, LL, I32, I32, P, I32, P, F, P, P, LL, P]),
-        "sg_paged_attention_rows": (I32, [KV, P, LL, I32, I32, P, I32, I32, P, P, F, P, P, LL, P]),
+        "sg_paged_attention_rows": (I32, [KV, P, LL, I32, I32, P, I32, I32, P, P, I32, F, P, P, LL, P]),
     }
     for name, (res, args) in sigs.items():
         fn = getattr(lib, name)

@@ -55,7 +55,8 @@ class PagedAttention:
         stream; token t is the positions[t]-th of page_table row rows[t] (row
         t if None; several tokens of a row in one call see each other's keys
         up to their own place).  A negative position marks a padding token,
-        whose row may be anything.  A row outside the table attends nothing;
+        whose row may be anything.  A token whose row lies outside the table,
+        or whose position outside ``rope``, attends nothing;
         ``ops.device_status`` reports it.  Returns (the attention's output [T,
         H], the new residual [T, H])."""
         T, D, kv = x.shape[0], self.cache.head_dim, self.cache.kv_heads
@@ -64,7 +65,8 @@ class PagedAttention:
         q, k, v = qkv.split([self.q_heads, kv, kv], dim=1)
         q = ops.append_kv(self.cache, q, k, v, page_table, positions, self.rope, rows=rows, q_weight=self.q_norm,
                           k_weight=self.k_norm, eps=self.eps)
-        o = ops.paged_attention(self.cache, q, page_table, positions + 1, rows=rows)
+        o = ops.paged_attention(self.cache, q, page_table, positions + 1, rows=rows,
+                                max_length=None if self.rope is None else self.rope.shape[0])
         o8, scales = ops.quantize_fp8(o.view(T, self.q_heads * D))
         return ops.fp8_linear(o8, scales, *self.out), residual
 

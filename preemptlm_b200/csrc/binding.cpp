@@ -6,6 +6,8 @@
 // way to it.  A C-ABI status other than SG_OK is returned as an int.
 #include <Python.h>
 
+#include <algorithm>
+
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -265,9 +267,9 @@ PyObject* append_kv(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
-// paged_attention(cache address, device, q, page_table, lengths, scale, rows): out
+// paged_attention(cache address, device, q, page_table, lengths, scale, rows, max_length): out
 PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  if (!want(n, 7, "paged_attention")) return nullptr;
+  if (!want(n, 8, "paged_attention")) return nullptr;
   return guarded([&]() -> PyObject* {
     const sg_kv_cache* c = cache_at(a[0]);
     const int64_t device = device_of(a[1]), D = c->head_dim;
@@ -278,6 +280,12 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (scale == -1.0 && PyErr_Occurred()) throw Raised();
     at::Tensor row_of;
     if (!is_none(a[6])) row_of = vector_int32(a[6], "rows", B, device);
+    int64_t max_length = INT32_MAX;
+    if (!is_none(a[7])) {
+      max_length = PyLong_AsLongLong(a[7]);
+      if (max_length == -1 && PyErr_Occurred()) throw Raised();
+      if (max_length < 0) value_error("max_length must not be negative");
+    }
     const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(device));
     const long long bytes = p_work_bytes(c, checked_int(B), checked_int(Hq));
     if (bytes < 0) return status(static_cast<int>(bytes));
@@ -285,8 +293,9 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     at::Tensor work = at::empty({bytes}, q.options().dtype(at::kByte));
     const int st = p_paged_attention(c, at_ptr<uint16_t>(q), q.stride(0), checked_int(B), checked_int(Hq),
                                      at_ptr<int32_t>(table), checked_int(table.size(0)), checked_int(table.size(1)),
-                                     at_ptr<int32_t>(row_of), at_ptr<int32_t>(lengths), static_cast<float>(scale),
-                                     at_ptr<uint16_t>(out), work.data_ptr(), bytes, stream(device));
+                                     at_ptr<int32_t>(row_of), at_ptr<int32_t>(lengths),
+                                     static_cast<int>(std::min<int64_t>(max_length, INT32_MAX)),
+                                     static_cast<float>(scale), at_ptr<uint16_t>(out), work.data_ptr(), bytes, stream(device));
     return st != SG_OK ? status(st) : wrap(out);
   });
 }

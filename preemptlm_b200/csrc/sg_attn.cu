@@ -205,6 +205,7 @@ struct Args {
   int table_rows;
   const int32_t* rows;  // [B] or null: row b's table row is b
   const int32_t* lengths;
+  int max_length;
   float scale_log2;  // softmax scale * log2(e)
   uint16_t* out;     // [B, q_heads, D]
   int32_t* prefix;   // [B + 1] first slice of each row on the line, then slices per warp
@@ -324,11 +325,11 @@ __device__ __forceinline__ bool no_row(const Args& a, int b) {
   return a.rows && static_cast<unsigned>(a.rows[b]) >= static_cast<unsigned>(a.table_rows);
 }
 
-// Tokens of row b that count; none if it has no row in the table.
+// Tokens of row b that count; none if it has no row in the table or is longer than allowed.
 __device__ __forceinline__ int row_length(const Args& a, int b) {
   const int cap = a.width << a.c.page_shift;
-  const int len = min(max(a.lengths[b], 0), cap);
-  return no_row(a, b) ? 0 : len;
+  const int n = a.lengths[b], len = min(max(n, 0), cap);
+  return n > a.max_length || no_row(a, b) ? 0 : len;
 }
 
 template <int SLICE>
@@ -445,6 +446,7 @@ attention_kernel(const Args a) {
       const int len = a.lengths[b];
       if (len > (a.width << a.c.page_shift)) record(SG_ERR_CAPACITY);
       if (len > 0 && no_row(a, b)) record(SG_ERR_CAPACITY);
+      if (len > a.max_length) record(SG_ERR_SHAPE);
       at += (row_length(a, b) + SLICE - 1) / SLICE * heads;
     }
     if (threadIdx.x == 0) a.prefix[a.B] = per;
@@ -1083,14 +1085,14 @@ extern "C" long long sg_paged_attention_work_bytes(const sg_kv_cache* cache, int
 
 extern "C" int sg_paged_attention_rows(const sg_kv_cache* cache, const uint16_t* q, long long q_stride, int B, int q_heads,
                                        const int32_t* page_table, int table_rows, int table_width, const int32_t* rows,
-                                       const int32_t* lengths, float scale, uint16_t* out, void* work,
+                                       const int32_t* lengths, int max_length, float scale, uint16_t* out, void* work,
                                        long long work_bytes, void* stream) {
   using namespace sg::attn;
   const long long need = sg_paged_attention_work_bytes(cache, B, q_heads);
   if (need < 0) return (int)need;
   Args a{};
   check_cache(cache, &a.c);
-  if (table_rows < 0 || table_width < 0) return SG_ERR_INVALID_ARG;
+  if (table_rows < 0 || table_width < 0 || max_length < 0) return SG_ERR_INVALID_ARG;
   if (q_stride % 8 || q_stride < 0) return SG_ERR_SHAPE;
   if (!rows && table_rows < B) return SG_ERR_INVALID_ARG;
   if (B == 0) return SG_OK;
@@ -1103,7 +1105,7 @@ extern "C" int sg_paged_attention_rows(const sg_kv_cache* cache, const uint16_t*
   const long long longest = static_cast<long long>(table_width) << a.c.page_shift;
   if (longest > (1 << 30) || B * heads * ((longest + 15) / 16) > (1 << 30)) return SG_ERR_SHAPE;
   a.q = q; a.q_stride = q_stride; a.B = B; a.q_heads = q_heads; a.width = table_width;
-  a.table = page_table; a.table_rows = table_rows; a.rows = rows; a.lengths = lengths; a.scale_log2 = scale * 1.44269504f; a.out = out;
+  a.table = page_table; a.table_rows = table_rows; a.rows = rows; a.lengths = lengths; a.max_length = max_length; a.scale_log2 = scale * 1.44269504f; a.out = out;
   int dev = 0;
   SG_CUDA_TRY(cudaGetDevice(&dev));
   return by_format(cache->head_dim, cache->bits, half, [&](auto dim, auto fp8, auto hf) -> int {
@@ -1114,6 +1116,6 @@ extern "C" int sg_paged_attention_rows(const sg_kv_cache* cache, const uint16_t*
 extern "C" int sg_paged_attention(const sg_kv_cache* cache, const uint16_t* q, long long q_stride, int B, int q_heads,
                                   const int32_t* page_table, int table_width, const int32_t* lengths, float scale,
                                   uint16_t* out, void* work, long long work_bytes, void* stream) {
-  return sg_paged_attention_rows(cache, q, q_stride, B, q_heads, page_table, B, table_width, nullptr, lengths, scale, out,
-                                 work, work_bytes, stream);
+  return sg_paged_attention_rows(cache, q, q_stride, B, q_heads, page_table, B, table_width, nullptr, lengths, INT32_MAX, scale,
+                                 out, work, work_bytes, stream);
 }

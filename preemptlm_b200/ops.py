@@ -450,17 +450,20 @@ def append_kv(cache, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, page_tab
 
 
 def paged_attention(cache, q: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor,
-                    scale: float | None = None, rows: torch.Tensor | None = None) -> torch.Tensor:
+                    scale: float | None = None, rows: torch.Tensor | None = None,
+                    max_length: int | None = None) -> torch.Tensor:
     """Attention of new tokens over the paged cache (``sg_paged_attention_rows``):
     row b of q [B, q_heads, D] attends the first lengths[b] (int32) cached
     tokens of row ``rows[b]`` (int32; row b if None) of page_table int32 [rows,
     pages] (at least B rows if ``rows`` is None); query heads share key-value heads in consecutive groups.  scale
     defaults to D ** -0.5.  Returns bf16 [B, q_heads, D]; a row of length 0 is
-    zero, and so is one outside the table.  The lengths stay on the device: a
+    zero, and so is one outside the table or, with ``max_length``, longer than
+    that (reported by ``device_status``).  The lengths stay on the device: a
     captured graph serves growing caches.  Several new tokens of one sequence
     are several rows of q with its table row and growing lengths."""
     return _result(_abi.native().paged_attention(cache.address, cache.index, q, page_table, lengths,
-                                                 cache.head_dim ** -0.5 if scale is None else scale, rows),
+                                                 cache.head_dim ** -0.5 if scale is None else scale, rows,
+                                                 max_length),
                    "sg_paged_attention_rows", 2)
 
 

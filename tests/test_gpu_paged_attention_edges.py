@@ -109,3 +109,38 @@ def test_table_with_more_rows_than_tokens():
     want, _ = att(x, r, table[:2], pos)
     got, _ = att(x, r, table, pos)
     assert torch.equal(got, want)
+
+
+def test_positions_past_the_rotation_table():
+    """A token whose position the append leaves out attends nothing, as a padding token does."""
+    att = make(256, 4, 2, 64, 64, 16, 64, BF)
+    att.cache.v.fill_(1.0)  # what a slot that was never written may hold
+    table = torch.arange(64, device=DEV, dtype=torch.int32).view(2, 32)
+    x, r = rand((2, 256), 1), rand((2, 256), 2, 2.0)
+    last = att.rope.shape[0] - 1
+    ops.device_status()
+    for pos in (last + 1, last + 100, (1 << 31) - 1):
+        at = torch.tensor([5, pos], dtype=torch.int32, device=DEV)
+        got, _ = att(x, r, table, at)
+        assert ops.device_status() == _abi.SG_ERR_SHAPE
+        assert bool((got[1] == 0).all()) and bool(got[0].any())
+    got, _ = att(x, r, table, torch.tensor([5, last], dtype=torch.int32, device=DEV))
+    assert ops.device_status() == 0 and bool(got[1].any())
+
+
+def test_rows_longer_than_the_limit():
+    page = 16
+    lengths = [40, 41, 39, 100, 0]
+    table, total = make_table(lengths, page, 1)
+    cache = make_cache(total, 2, page, 64, 16, 2)
+    q, n = rand((5, 4, 64), 3), torch.tensor(lengths, dtype=torch.int32, device=DEV)
+    ops.device_status()
+    want = ops.paged_attention(cache, q, table, n)
+    for most in (100, 1 << 40):
+        assert torch.equal(ops.paged_attention(cache, q, table, n, max_length=most), want)
+    assert ops.device_status() == 0
+    got = ops.paged_attention(cache, q, table, n, max_length=40)
+    assert ops.device_status() == _abi.SG_ERR_SHAPE
+    assert torch.equal(got[[0, 2, 4]], want[[0, 2, 4]]) and bool((got[[1, 3]] == 0).all())
+    with pytest.raises(ValueError):
+        ops.paged_attention(cache, q, table, n, max_length=-1)
