@@ -390,7 +390,9 @@ int sg_append_kv(const sg_kv_cache* cache, const uint16_t* q, long long q_stride
  * same pages and growing lengths.  A row of length 0 (or less) is zero; tokens
  * whose table entry is not a page of the cache are left out, and lengths past the
  * table are cut, both recorded (SG_ERR_CAPACITY; sg_device_status).  Lengths are
- * read on the device only.  work: sg_paged_attention_work_bytes() bytes, 16-byte
+ * read on the device only.  A table row holds at most 2^30 tokens, and 2^34 of all
+ * key-value heads together (a head counts once for every 16 query heads that share
+ * it).  work: sg_paged_attention_work_bytes() bytes, 16-byte
  * aligned, any contents; calls that overlap in time need one each. */
 long long sg_paged_attention_work_bytes(const sg_kv_cache* cache, int B, int q_heads);
 int sg_paged_attention(const sg_kv_cache* cache, const uint16_t* q, long long q_stride, int B, int q_heads,

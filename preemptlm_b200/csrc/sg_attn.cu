@@ -1,5 +1,6 @@
 // Paged key-value cache: the append (head norm, position rotation, write) and
 // the attention of new tokens over the cached ones.
+#include <algorithm>
 #include <type_traits>
 
 #include "sg_fp8.cuh"
@@ -1103,13 +1104,31 @@ extern "C" int sg_paged_attention_rows(const sg_kv_cache* cache, const uint16_t*
   const bool half = a.group <= 8;
   const long long heads = static_cast<long long>(a.c.kv_heads) * ((a.group + (half ? 7 : 15)) / (half ? 8 : 16));
   const long long longest = static_cast<long long>(table_width) << a.c.page_shift;
-  if (longest > (1 << 30) || B * heads * ((longest + 15) / 16) > (1 << 30)) return SG_ERR_SHAPE;
-  a.q = q; a.q_stride = q_stride; a.B = B; a.q_heads = q_heads; a.width = table_width;
+  const long long slices = heads * ((longest + 15) / 16);  // of a row, at most
+  if (longest > (1 << 30) || slices > (1 << 30)) return SG_ERR_SHAPE;
+  a.q = q; a.q_stride = q_stride; a.q_heads = q_heads; a.width = table_width;
   a.table = page_table; a.table_rows = table_rows; a.rows = rows; a.lengths = lengths; a.max_length = max_length; a.scale_log2 = scale * 1.44269504f; a.out = out;
   int dev = 0;
   SG_CUDA_TRY(cudaGetDevice(&dev));
+  // A line's slices are counted in 32 bits: where the table could hold more, as many
+  // rows at a time as fit, one after the other over the same work area.
+  const int most = static_cast<int>(std::min<long long>(B, (1 << 30) / std::max<long long>(slices, 1)));
   return by_format(cache->head_dim, cache->bits, half, [&](auto dim, auto fp8, auto hf) -> int {
-    return launch_attention<dim.value, fp8.value, hf.value>(a, static_cast<uint8_t*>(work), dev, (cudaStream_t)stream);
+    for (int b = 0; b < B; b += a.B) {
+      a.B = std::min(most, B - b);
+      const int st = launch_attention<dim.value, fp8.value, hf.value>(a, static_cast<uint8_t*>(work), dev, (cudaStream_t)stream);
+      if (st != SG_OK) return st;
+      a.q += a.B * q_stride;
+      a.out += static_cast<long long>(a.B) * q_heads * dim.value;
+      a.lengths += a.B;
+      if (rows) {
+        a.rows += a.B;
+      } else {
+        a.table += static_cast<long long>(a.B) * table_width;
+        a.table_rows -= a.B;
+      }
+    }
+    return SG_OK;
   });
 }
 

@@ -144,3 +144,35 @@ def test_rows_longer_than_the_limit():
     assert torch.equal(got[[0, 2, 4]], want[[0, 2, 4]]) and bool((got[[1, 3]] == 0).all())
     with pytest.raises(ValueError):
         ops.paged_attention(cache, q, table, n, max_length=-1)
+
+
+@pytest.mark.parametrize("shared", [True, False])
+def test_wide_tables(shared):
+    """Far more tokens in the table than in the rows: rows go by their lengths, around the cuts of the call too."""
+    heads, page, D, width = 32, 16, 64, 8192 if shared else 20000
+    B = 4500 if shared else 1900  # of 131072 (320000) tokens and 32 heads: 1.2e9 slices of 16
+    n = torch.arange(B, device=DEV, dtype=torch.int32) * 37 % 41
+    cache = make_cache(64, heads, page, D, 16, 2)
+    table = torch.full((3 if shared else B, width), -1, dtype=torch.int32, device=DEV)
+    table[:, :3] = torch.randint(64, (table.shape[0], 3), generator=torch.Generator(device=DEV).manual_seed(1), device=DEV)
+    rows = torch.arange(B, device=DEV, dtype=torch.int32) % 3 if shared else None
+    q = rand((B, heads, D), 3)
+    got = ops.paged_attention(cache, q, table, n, rows=rows)
+    narrow = table[:, :3].contiguous()
+    most = (1 << 30) // (heads * width)  # rows that are counted at a time
+    assert most < B
+    for first in (0, most - 25, B - 50):
+        at = slice(first, first + 50)
+        pages = narrow[at] if rows is None else narrow[rows[at].long()]
+        check_attention(got[at], *attend64(cache, q[at], pages, n[at].tolist()), 16)
+
+
+def test_longest_tables():
+    """One row of the widest table that is taken."""
+    cache = make_cache(8, 16, 1024, 64, 16, 2)
+    table = torch.full((1, 1 << 20), -1, dtype=torch.int32, device=DEV)  # 2^30 tokens
+    table[0, :4] = torch.tensor([3, 1, 7, 0])
+    q, n = rand((1, 16, 64), 3), torch.tensor([4000], dtype=torch.int32, device=DEV)
+    check_attention(ops.paged_attention(cache, q, table, n), *attend64(cache, q, table[:, :4], [4000]), 16)
+    with pytest.raises(_abi.SlottedGLUError):
+        ops.paged_attention(cache, q, torch.cat((table, table), dim=1), n)
