@@ -199,13 +199,17 @@ PyObject* fp8_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// Elements between tokens; a single token's stride says nothing (and contiguous()
+// leaves it as it is).
+int64_t token_stride(const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1) * t.size(2); }
+
 // [T, heads, D] bf16 whose heads are contiguous and whose tokens lie a multiple of
 // 16 bytes apart (a view of a wider row as it is), else a copy
 at::Tensor heads(PyObject* o, const char* name, int64_t D, int64_t device) {
   const at::Tensor& t = tensor(o, name);
   if (t.scalar_type() != at::kBFloat16 || t.dim() != 3 || t.size(2) != D || !on(t, device))
     type_error("%s must be a bf16 [T, heads, %lld] tensor on the cache's device", name, D);
-  if (t.stride(2) != 1 || (t.size(1) > 1 && t.stride(1) != D) || t.stride(0) % 8 || t.stride(0) < 0 || misaligned(t))
+  if (t.stride(2) != 1 || (t.size(1) > 1 && t.stride(1) != D) || token_stride(t) % 8 || token_stride(t) < 0 || misaligned(t))
     return packed(t);
   return t;
 }
@@ -257,7 +261,7 @@ PyObject* append_kv(PyObject*, PyObject* const* a, Py_ssize_t n) {
     at::Tensor out = at::empty({T, q.size(1), D}, q.options());
     const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(device));
     const int st = p_append_kv(
-        c, at_ptr<uint16_t>(q), q.stride(0), at_ptr<uint16_t>(k), k.stride(0), at_ptr<uint16_t>(v), v.stride(0),
+        c, at_ptr<uint16_t>(q), token_stride(q), at_ptr<uint16_t>(k), token_stride(k), at_ptr<uint16_t>(v), token_stride(v),
         checked_int(T), checked_int(q.size(1)), at_ptr<int32_t>(table), checked_int(table.size(0)),
         checked_int(table.size(1)), at_ptr<int32_t>(row_of), at_ptr<int32_t>(positions), at_ptr<float>(rope),
         rope.defined() ? checked_int(rope.size(1)) : 0, rope.defined() ? checked_int(rope.size(0)) : 0,
@@ -291,7 +295,7 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (bytes < 0) return status(static_cast<int>(bytes));
     at::Tensor out = at::empty({B, Hq, D}, q.options());
     at::Tensor work = at::empty({bytes}, q.options().dtype(at::kByte));
-    const int st = p_paged_attention(c, at_ptr<uint16_t>(q), q.stride(0), checked_int(B), checked_int(Hq),
+    const int st = p_paged_attention(c, at_ptr<uint16_t>(q), token_stride(q), checked_int(B), checked_int(Hq),
                                      at_ptr<int32_t>(table), checked_int(table.size(0)), checked_int(table.size(1)),
                                      at_ptr<int32_t>(row_of), at_ptr<int32_t>(lengths),
                                      static_cast<int>(std::min<int64_t>(max_length, INT32_MAX)),

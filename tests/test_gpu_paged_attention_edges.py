@@ -5,7 +5,7 @@ the ordinary cases."""
 import pytest
 import torch
 
-from preemptlm_b200 import _abi, ops
+from preemptlm_b200 import PagedKVCache, _abi, ops
 
 from .test_gpu_decoder_layer import make
 from .test_gpu_paged_attention import BF, DEV, attend64, check_attention, make_cache, make_table, rand
@@ -176,3 +176,21 @@ def test_longest_tables():
     check_attention(ops.paged_attention(cache, q, table, n), *attend64(cache, q, table[:, :4], [4000]), 16)
     with pytest.raises(_abi.SlottedGLUError):
         ops.paged_attention(cache, q, torch.cat((table, table), dim=1), n)
+
+
+@pytest.mark.parametrize("T", [0, 1, 2])
+@pytest.mark.parametrize("width", [257, 260, 264])
+def test_views_of_few_tokens(T, width):
+    """Rows of a wider buffer, whatever its width: read in place, or copied, with one token as with two."""
+    page, D = 16, 64
+    views = [rand((3, width), 10 + i)[:, : h * D].view(3, h, D)[:T] for i, h in enumerate((4, 2, 2))]
+    table = torch.arange(2, device=DEV, dtype=torch.int32).view(2, 1)
+    pos = torch.full((T,), 3, dtype=torch.int32, device=DEV)
+    out = []
+    for q, k, v in (views, [x.reshape(x.numel()).clone().view(x.shape) for x in views]):
+        cache = PagedKVCache.empty(2, 2, page, D)
+        rotated = ops.append_kv(cache, q, k, v, table, pos, None)
+        out.append((rotated, ops.paged_attention(cache, q, table, pos + 1), cache.k, cache.v))
+    for a, b in zip(*out):
+        assert torch.equal(a, b)
+    assert out[0][0].shape == (T, 4, D) and ops.device_status() == 0
