@@ -194,3 +194,20 @@ def test_views_of_few_tokens(T, width):
     for a, b in zip(*out):
         assert torch.equal(a, b)
     assert out[0][0].shape == (T, 4, D) and ops.device_status() == 0
+
+
+@pytest.mark.parametrize("shape", [(1, 2, 16, 64), (4, 1, 16, 64), (4, 2, 1, 64), (1, 1, 1, 64)])
+def test_cache_axes_of_one(shape):
+    """The stride of an axis of one is no reason to refuse a cache, nor to tell keys and values apart."""
+    k, v = rand(shape, 1), rand(shape, 2)
+    strides = lambda odd: [s if n > 1 else odd for s, n in zip(k.stride(), shape)]  # noqa: E731
+    want, got = PagedKVCache(k.clone(), v.clone()), PagedKVCache(k.as_strided(shape, strides(13)), v.as_strided(shape, strides(7)))
+    q = rand((1, 4, 64), 3)
+    x = rand((1, shape[1], 64), 4)
+    table = torch.zeros((1, 1), dtype=torch.int32, device=DEV)
+    at = torch.zeros(1, dtype=torch.int32, device=DEV)
+    out = [(ops.append_kv(c, q, x, x, table, at, None), ops.paged_attention(c, q, table, at + 1), c.k, c.v) for c in (want, got)]
+    for a, b in zip(*out):
+        assert torch.equal(a, b)
+    with pytest.raises(ValueError):
+        PagedKVCache(rand((4, 2, 16, 64), 1).transpose(1, 2), rand((4, 16, 2, 64), 1))
