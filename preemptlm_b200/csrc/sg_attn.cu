@@ -43,7 +43,9 @@ struct AppendArgs {
 // neighbouring ones past the rotated values), D / 16 lanes a row, and the same
 // chunks of HPT heads of its token, so cosines and sines are read once for
 // them.  Norm sums, the norm and the rotation are in fp32, with one rounding at the
-// store; an 8-bit value is the product with 1 / scale, rounded once more.
+// store; an 8-bit value is value / scale in fp32, rounded to e4m3 (a true division:
+// the codes then equal the definition's, where the product with 1 / scale is one
+// rounding more).
 // Bound by latency at decode sizes (one head a lane: as many lanes as there are)
 // and at prompt sizes by the bytes of the rows and the lanes in flight for them:
 // an 8191-token prompt of 40 heads of 128 into an 8-bit cache 33.8 us (163 MB, 4.8
@@ -152,12 +154,9 @@ __global__ void __launch_bounds__(256, 3) append_kv_kernel(const AppendArgs a) {
       const int kvh = is_v ? head - a.q_heads - a.c.kv_heads : head - a.q_heads;
       uint8_t* dst = (is_v ? a.c.v : a.c.k) + place + kvh * a.c.head_stride;
       if constexpr (FP8) {
-        const float inv = 1.0f / (is_v ? a.c.v_scale : a.c.k_scale)[kvh];
-        const uint64_t i2 = f2(inv, inv);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) x[k] = f2_mul(x[k], i2), y[k] = f2_mul(y[k], i2);
-        *reinterpret_cast<uint2*>(dst + da) = fp8_pack8(x);
-        *reinterpret_cast<uint2*>(dst + db) = fp8_pack8(y);
+        const float scale = (is_v ? a.c.v_scale : a.c.k_scale)[kvh];
+        *reinterpret_cast<uint2*>(dst + da) = fp8_pack8(x, scale);
+        *reinterpret_cast<uint2*>(dst + db) = fp8_pack8(y, scale);
       } else {
         *reinterpret_cast<uint4*>(dst + da * 2) = pack8(x);
         *reinterpret_cast<uint4*>(dst + db * 2) = pack8(y);

@@ -81,9 +81,9 @@ __device__ __forceinline__ uint4 pack8(const uint64_t (&v)[4]) {
   const float2 a = f2_get(v[0]), b = f2_get(v[1]), c = f2_get(v[2]), d = f2_get(v[3]);
   return make_uint4(bf16_pair(a.x, a.y), bf16_pair(b.x, b.y), bf16_pair(c.x, c.y), bf16_pair(d.x, d.y));
 }
-__device__ __forceinline__ uint2 fp8_pack8(const uint64_t (&v)[4]) {
+__device__ __forceinline__ uint2 fp8_pack8(const uint64_t (&v)[4], float s) {
   const float2 a = f2_get(v[0]), b = f2_get(v[1]), c = f2_get(v[2]), d = f2_get(v[3]);
-  return make_uint2(fp8_pair(a.x, a.y) | fp8_pair(b.x, b.y) << 16, fp8_pair(c.x, c.y) | fp8_pair(d.x, d.y) << 16);
+  return fp8_pack8({a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y}, s);
 }
 
 }  // namespace sg

@@ -8,7 +8,7 @@ import torch
 from preemptlm_b200 import PagedKVCache, _abi, ops
 
 from .test_gpu_decoder_layer import make
-from .test_gpu_paged_attention import BF, DEV, attend64, check_attention, make_cache, make_table, rand
+from .test_gpu_paged_attention import BF, DEV, F8, attend64, check_attention, make_cache, make_table, rand
 
 pytestmark = pytest.mark.gpu
 
@@ -211,3 +211,51 @@ def test_cache_axes_of_one(shape):
         assert torch.equal(a, b)
     with pytest.raises(ValueError):
         PagedKVCache(rand((4, 2, 16, 64), 1).transpose(1, 2), rand((4, 16, 2, 64), 1))
+
+
+@pytest.mark.parametrize("Hq,Hkv,D,T", [(4, 2, 64, 300), (8, 4, 128, 300), (2, 3, 256, 300), (2, 24, 128, 2400)])
+def test_append_codes_equal_the_definition(Hq, Hkv, D, T):
+    """An 8-bit cache holds e4m3(value / scale), the quotient in fp32, code for code; the last size has several heads a lane.
+    Keys are neither normed nor rotated here."""
+    page = 16
+    cache = PagedKVCache.empty(-(-T // page), Hkv, page, D, F8, *(
+        0.005 + 0.1 * torch.rand(Hkv, generator=torch.Generator(device=DEV).manual_seed(i), device=DEV) for i in (1, 2)))
+    q, k, v = rand((T, Hq, D), 3), rand((T, Hkv, D), 4), rand((T, Hkv, D), 5)
+    table = torch.arange(-(-T // page), device=DEV, dtype=torch.int32)[None]
+    pos = torch.arange(T, device=DEV, dtype=torch.int32)
+    ops.append_kv(cache, q, k, v, table, pos, None, rows=torch.zeros_like(pos))
+    for c, x, s in ((cache.k, k, cache.k_scale), (cache.v, v, cache.v_scale)):
+        got = c.view(torch.uint8).transpose(1, 2).flatten(0, 1)[:T]
+        want = (x.float() / s[:, None]).clamp(-448, 448).to(F8).view(torch.uint8)
+        assert torch.equal(got, want), int((got != want).sum())
+
+
+def test_append_with_the_smallest_scales():
+    """Zeros stay zeros and values saturate, at scales whose reciprocal is no fp32 number."""
+    scale = torch.tensor([1e-39, 1e-45], device=DEV)
+    cache = PagedKVCache.empty(1, 2, 16, 64, F8, scale, scale)
+    k = torch.zeros((1, 2, 64), dtype=BF, device=DEV)
+    k[0, :, 0] = 1.0
+    table = torch.zeros((1, 1), dtype=torch.int32, device=DEV)
+    ops.append_kv(cache, k, k, -k, table, table[0], None)
+    for c, top in ((cache.k, 448), (cache.v, -448)):
+        got = c[0, :, 0].float()
+        assert bool((got[:, 0] == top).all()) and bool((got[:, 1:] == 0).all())
+
+
+def test_append_rounds_ties_to_even():
+    """Values that are a middle of two e4m3 numbers times the scale: the quotient is that middle, and goes to the even one."""
+    page, D, T = 16, 128, 64
+    scale = torch.tensor([3.0, 5.0, 7.0, 0.625], device=DEV)  # three bits: the product with a middle's five is a bf16 value
+    cache = PagedKVCache.empty(T // page, 4, page, D, F8, scale, scale)
+    r = torch.Generator().manual_seed(1)
+    middle = (2 * torch.randint(8, 16, (T, 4, D), generator=r) + 1) * 2.0 ** torch.randint(-8, 4, (T, 4, D), generator=r)
+    v = (middle.to(DEV) * scale[:, None]).to(BF)
+    assert torch.equal(v.double() / scale.double()[:, None], middle.to(DEV).double())
+    table = torch.arange(T // page, device=DEV, dtype=torch.int32)[None]
+    pos = torch.arange(T, device=DEV, dtype=torch.int32)
+    ops.append_kv(cache, v, v, v, table, pos, None, rows=torch.zeros_like(pos))
+    want = middle.to(F8).view(torch.uint8).to(DEV)
+    for c in (cache.k, cache.v):
+        got = c.view(torch.uint8).transpose(1, 2).flatten(0, 1)
+        assert torch.equal(got, want), int((got != want).sum())
