@@ -18,11 +18,6 @@ from . import _abi
 KV_DTYPES = {torch.bfloat16: 16, torch.float8_e4m3fn: 8}
 
 
-def _strides(t: torch.Tensor) -> tuple[int, ...]:
-    """Strides, 0 for an axis of one (its stride says nothing)."""
-    return tuple(s if n > 1 else 0 for s, n in zip(t.stride(), t.shape))
-
-
 class PagedKVCache:
     """Views of a layer's key and value pages, [pages, kv_heads, page_size,
     head_dim] each, bf16 or e4m3 (``float8_e4m3fn``).
@@ -38,8 +33,12 @@ class PagedKVCache:
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor | None = None,
                  v_scale: torch.Tensor | None = None):
-        shape, strides, dtype, index = k.shape, _strides(k), k.dtype, k.get_device()
-        if len(shape) != 4 or v.shape != shape or v.dtype != dtype or _strides(v) != strides or v.get_device() != index:
+        shape, strides, dtype, index = k.shape, k.stride(), k.dtype, k.get_device()
+        same = v.stride() == strides
+        if 1 in shape:  # the stride of an axis of one says nothing
+            strides = tuple(0 if n == 1 else s for s, n in zip(strides, shape))
+            same = v.shape == shape and strides == tuple(0 if n == 1 else s for s, n in zip(v.stride(), shape))
+        if len(shape) != 4 or v.shape != shape or v.dtype != dtype or not same or v.get_device() != index:
             raise ValueError("k and v must be [pages, kv_heads, page_size, head_dim] tensors of one type and stride")
         bits = KV_DTYPES.get(dtype)
         if bits is None:
