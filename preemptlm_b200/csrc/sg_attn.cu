@@ -1051,8 +1051,11 @@ extern "C" int sg_append_kv(const sg_kv_cache* cache, const uint16_t* q, long lo
   a.rope = rope; a.rot = rot; a.max_pos = max_pos;
   a.q_weight = q_weight; a.k_weight = k_weight; a.eps = eps; a.q_out = q_out;
   const long long heads = q_heads + 2LL * a.c.kv_heads;
+  int dev = 0;
+  SG_CUDA_TRY(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64) return SG_ERR_CUDA;
   // four heads a lane once that still leaves every SM its fill of lanes
-  const bool four = T * heads * (D / 16) >= 4LL * 148 * 768;
+  const bool four = T * heads * (D / 16) >= 4LL * num_sms(dev) * 768;
   const long long blocks = (T * (four ? (heads + 3) / 4 : heads) * (D / 16) + 255) / 256;
   if (blocks > (1 << 23)) return SG_ERR_SHAPE;
   return by_format(D, cache->bits, false, [&](auto dim, auto fp8, auto) -> int {
