@@ -385,7 +385,8 @@ int sg_append_kv(const sg_kv_cache* cache, const uint16_t* q, long long q_stride
 
 /* out[b, hq] = softmax_j(scale * q[b, hq] . k[j, hq / group]) v[j, hq / group]
  * over the cached tokens j < lengths[b] of page_table row b; group = q_heads /
- * kv_heads.  q [B, q_heads, D] bf16, rows q_stride elements apart; out bf16
+ * kv_heads.  An infinite value in one of these tokens may come out as NaN (a probability
+ * is a sum of two parts).  q [B, q_heads, D] bf16, rows q_stride elements apart; out bf16
  * [B, q_heads, D].  Several new tokens of one sequence are several rows with the
  * same pages and growing lengths.  A row of length 0 (or less) is zero; tokens
  * whose table entry is not a page of the cache are left out, and lengths past the

@@ -3,8 +3,10 @@
 The operators between two expert layers, run together as a serving step runs
 them.  Every projection is 8-bit with block scales; the rows that enter one are
 brought to 8 bits by the kernel before it (the norm, or ``ops.quantize_fp8``).
-No host read anywhere, so a step can be captured as a CUDA graph.  No
-counterpart in the reference (its attention blocks are mlx_lm's).
+No host read anywhere, so a step can be captured as a CUDA graph.  A block with
+a gate on its output or projections in another format puts the single calls
+together itself.  No counterpart in the reference (its attention blocks are
+mlx_lm's).
 """
 
 from __future__ import annotations

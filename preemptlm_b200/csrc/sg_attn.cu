@@ -44,13 +44,16 @@ struct AppendArgs {
 // chunks of HPT heads of its token, so cosines and sines are read once for
 // them.  Norm sums, the norm and the rotation are in fp32, with one rounding at the
 // store; an 8-bit value is value / scale in fp32, rounded to e4m3 (a true division:
-// the codes then equal the definition's, where the product with 1 / scale is one
-// rounding more).
+// the codes then equal the definition's; the product with 1 / scale is one rounding
+// more, which sends middles the wrong way, and makes NaN of zeros where 1 / scale
+// overflows, for 33.1 us in place of 36.4 at the size below).
 // Bound by latency at decode sizes (one head a lane: as many lanes as there are)
 // and at prompt sizes by the bytes of the rows and the lanes in flight for them:
-// an 8191-token prompt of 40 heads of 128 into an 8-bit cache 33.8 us (163 MB, 4.8
-// TB/s) with four heads a lane, two of them loaded ahead, in 80 registers; 35.1
-// with two heads in 64, 41.6 with four loaded at once in 96, 43.5 with one.
+// an 8191-token prompt of 40 heads of 128, in a row of calls, into an 8-bit cache
+// 36.4 us (163 MB, 4.4 TB/s) with four heads a lane, two of them loaded ahead, in 80
+// registers, and into a bf16 one 34.5 (171 MB, 4.9 TB/s).  Other forms, with the
+// product in the 8-bit store, where this one took 33.8: two heads in 64 registers
+// 35.1, four loaded at once in 96 41.6, one head 43.5.
 template <int D, bool FP8, int HPT>
 __global__ void __launch_bounds__(256, 3) append_kv_kernel(const AppendArgs a) {
   constexpr int LP = D / 16;  // lanes per head row
@@ -169,7 +172,10 @@ __global__ void __launch_bounds__(256, 3) append_kv_kernel(const AppendArgs a) {
 //
 // o = softmax(scale q k^T) v of each row's query heads over its cached tokens.
 // The query heads that share a key-value head (8 or 16 of them a pass) meet
-// every key and value in registers, so the cache is read once for all of them;
+// every key and value in registers, so the cache is read once for all of them, or
+// once for every 16 of a larger group.  Every row of queries reads its tokens by
+// itself: made for one or a few new tokens of a sequence; the tokens of a prompt
+// work too, each over its whole prefix.  The
 // work per cached byte is small (2 to 8 flops), and the kernel is bound by the
 // cache's bytes from HBM.  That is why the products run on mma.sync: a tcgen05
 // product has at least 64 rows on its token side and keeps its scores in tensor
@@ -191,8 +197,8 @@ __global__ void __launch_bounds__(256, 3) append_kv_kernel(const AppendArgs a) {
 // and attention_combine_kernel joins the parts in the order of the tokens: the
 // result does not depend on timing.  Measured with the joining: 64 rows of 0 to 8192
 // tokens, 16 heads over 2 of 256, 90.6 us (537 MB, 0.91 of a copy's rate); one row of
-// 131071 48.9 us (0.84); 128 rows of 0 to 8000 over an 8-bit cache, 32 heads over 4
-// of 128, 94 us (0.85).
+// 131071 50.3 us (0.82); 128 rows of 0 to 8000 over an 8-bit cache, 32 heads over 4
+// of 128, 97.2 us (0.83; inputs change from pass to pass here, 93.5 where they stay).
 
 constexpr int WARPS = 4;
 
@@ -529,7 +535,9 @@ attention_kernel(const Args a) {
         sc[t][0] = sc[t][1] = a.scale_log2;
         if constexpr (FP8) {
           // f16 fragments of q / 2^e, 2^e the power of two of the row's largest
-          // magnitude: exact down to 2^-14 of it, and no overflow
+          // magnitude: no overflow, exact for bf16 values down to 2^-17 of 2^e, and off
+          // by 2^-25 of 2^e at most below that (e4m3 keys are exact in f16, not in a
+          // product with bf16 without as many instructions again to widen them)
           float v[D / 64][16];
           float top = 0.0f;
 #pragma unroll
@@ -833,10 +841,12 @@ attention_kernel(const Args a) {
 // Joins the parts that the warps left of a (row, head), in the order of the
 // tokens; rows without tokens become zeros.  A group of PIECE / 4 lanes (four
 // values each) walks the parts of PIECE values of one head.  The kernel is a chain
-// of a few L2 latencies, so its shape goes by how many parts a head can have:
-// many rows have few parts each, and one group walks them all (GROUPS 1); few
-// rows may have hundreds (one long row over the whole grid), and a block's GROUPS
-// groups walk a share each, joined in shared memory.
+// of a few L2 latencies: few (row, head)s may have hundreds of parts each (one long
+// row over the whole grid), and a block's GROUPS groups walk a share each, joined in
+// shared memory; many have few parts each, and one group walks them all (GROUPS 1).
+// How many parts a row really has, only the device knows: the host goes by the number
+// of (row, head)s, as if all rows were equally long.  One long row among many short ones
+// is joined by one group, four parts at a time.
 template <int D, int R, int SLICE, int PIECE, int GROUPS>
 __global__ void __launch_bounds__(GROUPS == 1 ? 128 : PIECE / 4 * GROUPS)
 attention_combine_kernel(const Args a) {
@@ -982,6 +992,11 @@ static int launch_attention(Args a, uint8_t* work, int dev, cudaStream_t s) {
     attr_done[dev] = true;
   }
   SG_CUDA_TRY(launch_after_previous(attention_kernel<D, FP8, HALF>, w.grid, WARPS * 32, C::SMEM, s, a));
+  // us with the joining, 32 groups / 16 / 4 / 1, by (row, head)s: 16 of 131071 tokens 49 /
+  // 51 / 77 / 160; 128 of 0 to 20000 16.2 / 16.8 / 31 / 81; 256 of 0 to 600 10.0 / 7.7 / 9.6
+  // / 20; 512 of 0 to 4000 22 / 16.5 / 17.9 / 31 (heads of 256 45 / 36 / 32 / 39); 1024 of 0
+  // to 8192 119 / 100 / 91 / 94; 2048 of 0 to 600 41 / 23 / 14.5 / 16.7; 4096 of 0 to 8000
+  // 153 / 113 / 96 / 94; 16384 of 0 to 1000 304 / 168 / 106 / 94.
   const long long rows = static_cast<long long>(a.B) * a.q_heads;
   constexpr int PIECE = D < 128 ? D : 128;
   if (rows <= 64) return launch_combine<D, C::R, C::SLICE, 32, 32>(a, s);

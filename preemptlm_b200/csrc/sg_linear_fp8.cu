@@ -32,7 +32,7 @@
 // Bound by the weights' bytes and a chain of latencies for few tokens (16 x 2048 x
 // 5120 6.4 us in a row of calls, 1.6 of it bytes), by the tensor cores and the
 // epilogue beside them for many (4096 x 4096 x 9216 152 us, 2.03 PFLOP/s, in a
-// short burst; 178 at the card's power cap).
+// short burst; 174 at the card's power cap).
 //
 // Every mbarrier wait is bounded; on expiry the CTA records SG_ERR_TIMEOUT, waits
 // (bounded) for its copies in flight, frees its tensor memory and returns.

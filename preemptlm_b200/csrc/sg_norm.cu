@@ -10,8 +10,9 @@ namespace sg {
 // 8-value chunks i, i + blockDim, ...; 16 neighbouring lanes hold one block of
 // 128, so its largest magnitude is four shuffles.  Bound by the rows' bytes: 8192 x
 // 4096 with the residual 41.8 us (268 MB, 6.4 TB/s, 0.98 of a copy's rate); one row is
-// a chain of two latencies, 1.6 us.  One chunk a thread up to 2048 values and two up
-// to 8192 keep 8 CTAs on an SM; longer rows take four.
+// a chain of two latencies, 1.6 us.  One chunk a thread up to 2048 values (26 to 29
+// registers, 8 CTAs of 256 on an SM), two up to 8192 (40: six CTAs of 256 at 4096
+// values, three of 512 at 8192), four beyond (about 50: up to 1024 threads, one CTA).
 template <int VPT, bool FP8>
 __global__ void __launch_bounds__(256 * VPT)
 add_rms_norm_kernel(const uint16_t* x, const uint16_t* residual,

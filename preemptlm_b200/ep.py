@@ -444,7 +444,8 @@ class ExpertParallelMoE:
 class ExpertParallelStack:
     """The MoE blocks of a decoder stack, each expert-parallel: L layers
     applied in turn to the residual stream, ``x <- x + layer(x)`` (the
-    attention blocks between them are outside this library).  The layers may
+    attention blocks between them, ``attention.PagedAttention`` or the host
+    model's, are not part of it).  The layers may
     share one peer exchange: they run one after another on the stream, so a
     rank's next send into a peer follows its wait for that peer's outputs of
     the layer before, as between two steps of one layer.  ``capture`` records

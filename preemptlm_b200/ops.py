@@ -460,7 +460,8 @@ def paged_attention(cache, q: torch.Tensor, page_table: torch.Tensor, lengths: t
     zero, and so is one outside the table or, with ``max_length``, longer than
     that (reported by ``device_status``).  The lengths stay on the device: a
     captured graph serves growing caches.  Several new tokens of one sequence
-    are several rows of q with its table row and growing lengths."""
+    are several rows of q with its table row and growing lengths; each reads
+    its whole prefix, so a prompt's time grows with the square of its length."""
     return _result(_abi.native().paged_attention(cache.address, cache.index, q, page_table, lengths,
                                                  cache.head_dim ** -0.5 if scale is None else scale, rows,
                                                  max_length),
